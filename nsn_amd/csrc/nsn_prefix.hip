@@ -45,6 +45,7 @@
 // both halves (17 KB of code, no spills) took it from 34.7 to 25.8 us, one fma
 // instead of a multiply and an fma and reads a step ahead to 24.3.
 #include "nsn_segment.hpp"
+#include "nsn_own_ranges.hpp"
 #include "nsn_tile.hpp"
 #include "nsn_unpack.hpp"
 #include "nsn_wave.hpp"
@@ -676,30 +677,11 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(2))
     const uint32_t hkv = static_cast<uint32_t>(p.heads_kv);
     const int b = static_cast<int>(blockIdx.x / hkv), kvh = static_cast<int>(blockIdx.x % hkv);
     // the sequence's own tokens: none where its counts do not fit the cache
-    int32_t T = p.seq_len[b], nk = p.k.blocks ? p.k.blocks[b] : 0, nv = p.v.blocks ? p.v.blocks[b] : 0;
-    auto fits = [&](const fast::FastSide &sd, int32_t nb) {
-        if (nb < 0 || nb > sd.block_cap) return false;
-        const int64_t rest = static_cast<int64_t>(T) - static_cast<int64_t>(nb) * kBlockTok;
-        return rest <= 0 || (sd.tail != nullptr && rest <= sd.tail_cap);
-    };
-    if (!fits(p.k, nk) || !fits(p.v, nv)) {
-        if (tid == 0 && kvh == 0) raise_status(p.status, NSN_ST_CAPACITY);
-        T = 0;
-    }
-    T = T > 0 ? T : 0;
-    // ranges of equal cost: a packed token 1, a dense one 3 (read without the
-    // prefetch); packed cuts at blocks, dense ones at 16 tokens
-    const int both = min(nk, nv);
-    const int packed = both > T / kBlockTok ? T : both * kBlockTok;
-    const int64_t cost = packed + 3 * static_cast<int64_t>(T - packed);
-    const int dense = nk == nv ? 16 : kBlockTok;   // (one side packed: still in blocks)
-    auto cut = [&](int k) {
-        const int64_t c = cost * k / kOwnWaves;
-        if (k == kOwnWaves) return T;
-        if (c <= packed) return static_cast<int>(c) / kBlockTok * kBlockTok;
-        const int d = (static_cast<int>((c - packed) / 3) + dense - 1) / dense * dense;   // (< T, to 64 above)
-        return d < T - packed ? packed + d : T;
-    };
+    const OwnRanges own(p.seq_len[b], p.k.blocks ? p.k.blocks[b] : 0, p.v.blocks ? p.v.blocks[b] : 0,
+                        {p.k.block_cap, p.k.tail ? p.k.tail_cap : 0},
+                        {p.v.block_cap, p.v.tail ? p.v.tail_cap : 0});
+    if (own.over && tid == 0 && kvh == 0) raise_status(p.status, NSN_ST_CAPACITY);
+    auto cut = [&](int k) { return own.cut(k, kOwnWaves); };
     int count = 0, slot = 0;   // (non-empty ranges, those before this wave's)
 #pragma unroll
     for (int k = 0; k < kOwnWaves; ++k) {
@@ -717,7 +699,8 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(2))
         if (cut(wave) < cut(wave + 1)) {
             const fast::Lds<BITS, GRP> sh{s_afrag[wave], s_pbuf[wave], s_k0[wave], s_k1[wave],
                                           s_v0[wave],    s_v1[wave],   s_m0[wave], s_m1[wave]};
-            fast::segment<BITS, QDT, false, GRP, TBF>(p, sh, b, kvh, cut(wave), cut(wave + 1), nk, nv, slot, count, l);
+            fast::segment<BITS, QDT, false, GRP, TBF>(p, sh, b, kvh, cut(wave), cut(wave + 1), own.nk, own.nv, slot, count,
+                                                       l);
         }
     } else {   // 2 * (kWaves - kOwnWaves) == kGroups groups of 32 lanes
         const int grp = (tid >> 5) - 2 * kOwnWaves, head = grp / per;
