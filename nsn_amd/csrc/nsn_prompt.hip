@@ -76,13 +76,16 @@ struct PromptParams {
 __device__ __forceinline__ int k_swz(int t) { return t & 15; }
 __device__ __forceinline__ int v_swz(int t) { return ((t & 3) << 2) | ((t >> 2) & 3); }
 
-// Sequence s as the kernel uses it: its first token and length; a sequence
-// whose offsets decrease or leave the token rows has none (and is flagged).
-__device__ __forceinline__ void sequence(const PromptParams &p, int s, int32_t &start, int32_t &n, bool &bad) {
+// Sequence s of the first `seqs` as the kernel uses it: its first token and
+// length; one whose offsets decrease or leave the token rows has none (and is flagged).
+__device__ __forceinline__ void sequence(const PromptParams &p, int s, int seqs, int32_t &start, int32_t &n, bool &bad,
+                                         bool &decreases) {
     start = n = 0;
-    if (s >= p.seqs) return;
+    decreases = false;
+    if (s >= seqs) return;
     const int32_t a = p.cu[s], b = p.cu[s + 1];
-    if (a < 0 || b < a || b > p.tokens) {
+    decreases = b < a;
+    if (a < 0 || decreases || b > p.tokens) {
         bad = true;
         return;
     }
@@ -94,27 +97,37 @@ __device__ __forceinline__ int32_t tiles_of(const PromptParams &p, int32_t n) {
 }
 
 // Tile t of all sequences' tiles, the last places first: its sequence's first
-// token and length and its place z.  False: no such tile.
+// token and length and its place z.  False: no such tile.  Sequences behind a
+// decrease of the offsets may repeat earlier ones' rows: they are left out, so
+// that no row has two tiles and the tiles are no more than the grid's.
 __device__ __forceinline__ bool find_tile(const PromptParams &p, int32_t t, bool first_wg, int32_t &start, int32_t &n,
                                           int32_t &z) {
     const int l = threadIdx.x & 63;
-    bool bad = false;
+    bool bad = false, decreases;
+    int seqs = p.seqs;
+    auto cut = [&](int s0, int32_t &m) {   // after sequences s0 + l: none from the first decrease on
+        const uint64_t at = __ballot(decreases);
+        if (at == 0) return;
+        seqs = s0 + __ffsll(static_cast<unsigned long long>(at)) - 1;
+        if (s0 + l >= seqs) m = 0;
+    };
     int32_t st0, n0;
-    sequence(p, l, st0, n0, bad);
+    sequence(p, l, seqs, st0, n0, bad, decreases);
+    cut(0, n0);
     const int32_t t0 = tiles_of(p, n0);
     int32_t top = wave_max(t0);
-    for (int s = 64; s < p.seqs; s += 64) {
+    for (int s = 64; s < seqs; s += 64) {
         int32_t a, m;
-        sequence(p, s + l, a, m, bad);
+        sequence(p, s + l, seqs, a, m, bad, decreases);
+        cut(s, m);
         top = max(top, wave_max(tiles_of(p, m)));
     }
     if (first_wg && __ballot(bad) && l == 0) raise_status(p.status, NSN_ST_CAPACITY);
     auto above = [&](int32_t place) {   // tiles at places >= place
         int32_t c = wave_sum(max(0, t0 - place));
-        for (int s = 64; s < p.seqs; s += 64) {
+        for (int s = 64; s < seqs; s += 64) {
             int32_t a, m;
-            bool b;
-            sequence(p, s + l, a, m, b);
+            sequence(p, s + l, seqs, a, m, bad, decreases);
             c += wave_sum(max(0, tiles_of(p, m) - place));
         }
         return c;
@@ -132,10 +145,9 @@ __device__ __forceinline__ bool find_tile(const PromptParams &p, int32_t t, bool
     }
     z = lo;
     int32_t r = t - fhi;   // the r-th sequence with more than z tiles
-    for (int s = 0;; s += 64) {
+    for (int s = 0; s < seqs; s += 64) {
         int32_t a = st0, m = n0;
-        bool b;
-        if (s) sequence(p, s + l, a, m, b);
+        if (s) sequence(p, s + l, seqs, a, m, bad, decreases);
         const uint64_t has = __ballot(tiles_of(p, m) > z);
         const int32_t c = __popcll(has);
         if (r >= c) {
@@ -148,6 +160,7 @@ __device__ __forceinline__ bool find_tile(const PromptParams &p, int32_t t, bool
         n = __builtin_amdgcn_readlane(m, lane);
         return true;
     }
+    return false;
 }
 
 // One tile.  LO (bf16): the softmax weights enter the PV product and the sums

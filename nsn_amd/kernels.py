@@ -594,8 +594,9 @@ def prompt_attention(q, k, v, cu_seqlens, *, scale=SCALE, status=None, check=Tru
     reaches the queries from it on only.  No gradient.  bf16 weights are
     rounded once, except for the first 64 queries of a sequence, whose few
     weights enter as hi + lo (~2^-17).  ``check`` reads the offsets and the
-    status word back and raises; without it offsets that decrease or leave
-    the rows set NSN_ST_CAPACITY in ``status`` and leave that sequence out.
+    status word back and raises; without it offsets that leave the rows set
+    NSN_ST_CAPACITY in ``status`` and leave that sequence out, offsets that
+    decrease that one and every sequence behind it.
 
     A prompt's queries see nothing of a cache: ``prefill_attention`` is the
     form over a packed context, ``StreamingKVCache.prompt`` this one with the
