@@ -39,6 +39,7 @@
 // workgroup finds its (sequence, place) from the offsets on the device.
 #include <type_traits>
 
+#include "nsn_rows.hpp"
 #include "nsn_tile.hpp"
 #include "nsn_wave.hpp"
 
@@ -163,13 +164,14 @@ __device__ __forceinline__ bool find_tile(const PromptParams &p, int32_t t, bool
     return false;
 }
 
-// One tile.  LO (bf16): the softmax weights enter the PV product and the sums
-// as bf16 hi + lo (~2^-17 relative) instead of one bf16 rounding, for the tiles
-// whose first queries attend a handful of tokens, where one weight's rounding
-// moves the output by up to 2^-9 of |v|.
+// One tile; true: it is to be done again, marked (written: this wave's rows
+// are out and stay).  LO (bf16): the softmax weights enter the PV product and the
+// sums as bf16 hi + lo (~2^-17 relative) instead of one bf16 rounding, for the
+// tiles whose first queries attend a handful of tokens, where one weight's
+// rounding moves the output by up to 2^-9 of |v|.
 template <int DT, bool LO>
 __device__ __forceinline__ bool attend_tile(const PromptParams &p, uint8_t (&stg)[kStages][2 * kHalf], int &again, int kvh,
-                                            int64_t start, int32_t n, int32_t z, bool marked) {
+                                            int64_t start, int32_t n, int32_t z, bool marked, bool &written) {
     int tid = threadIdx.x;
     asm volatile("" : "+v"(tid));   // (nothing of a tile is kept for its second time)
     asm volatile("" : "+s"(z));
@@ -398,10 +400,19 @@ __device__ __forceinline__ bool attend_tile(const PromptParams &p, uint8_t (&stg
         else output(j);
     }
 
-    // ---- O = O^T / sum
+    // ---- O = O^T / sum.  A wave with a value that is not finite writes nothing
+    // the first time: the output may lie in the queries' place, which it reads again.
     const float rl = 1.f / halves_sum(lsum);
     bool bad = false;
-    if (r < rows) {
+#pragma unroll
+    for (int ct = 0; ct < 4; ++ct)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            acc[ct][i] *= rl;
+            bad |= !finite(acc[ct][i]);
+        }
+    const bool redo = __builtin_amdgcn_ballot_w64(bad && r < rows) != 0;   // (uniform)
+    if (r < rows && (marked ? !written : !redo)) {
         int ro = r;   // (its query and head once more: kept across the blocks they cost a spill)
         asm volatile("" : "+v"(ro));
         const int qo = ro / G;
@@ -414,14 +425,9 @@ __device__ __forceinline__ bool attend_tile(const PromptParams &p, uint8_t (&stg
                 uint32_t w[2][2];
 #pragma unroll
                 for (int x = 0; x < 2; ++x) {
-                    float o[4];
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        o[i] = acc[ct][4 * (c + x) + i] * rl;
-                        bad |= !finite(o[i]);
-                    }
-                    w[x][0] = pk<DT>(o[0], o[1]);
-                    w[x][1] = pk<DT>(o[2], o[3]);
+                    const int i = 4 * (c + x);
+                    w[x][0] = pk<DT>(acc[ct][i], acc[ct][i + 1]);
+                    w[x][1] = pk<DT>(acc[ct][i + 2], acc[ct][i + 3]);
                 }
                 const auto a = __builtin_amdgcn_permlane32_swap(w[0][0], w[1][0], false, false);
                 const auto b = __builtin_amdgcn_permlane32_swap(w[0][1], w[1][1], false, false);
@@ -429,10 +435,11 @@ __device__ __forceinline__ bool attend_tile(const PromptParams &p, uint8_t (&stg
             }
     }
     if (marked) {
-        if (bad) raise_status(p.status, NSN_ST_NONFINITE_OUTPUT);
+        if (bad && r < rows && !written) raise_status(p.status, NSN_ST_NONFINITE_OUTPUT);
         return false;
     }
-    if (__builtin_amdgcn_ballot_w64(bad) != 0 && l == 0) again = 1;
+    written = !redo;
+    if (redo && l == 0) again = 1;
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     __builtin_amdgcn_s_barrier();   // (also: every wave has left the stages)
     asm volatile("" ::: "memory");
@@ -449,9 +456,10 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(2))
     if (!find_tile(p, static_cast<int32_t>(blockIdx.x / hkv), blockIdx.x == 0 && threadIdx.x < 64, start, n, z)) return;
     // queries up to the 64th: weights as hi + lo
     const bool first = DT == NSN_DTYPE_BF16 && static_cast<int64_t>(z) * kRows < static_cast<int64_t>(kBlockTok) * p.group;
+    bool written = false;
     for (bool marked = false, more = true; more; marked = true) {
-        if (first) more = attend_tile<DT, DT == NSN_DTYPE_BF16>(p, stg, again, kvh, start, n, z, marked);
-        else more = attend_tile<DT, false>(p, stg, again, kvh, start, n, z, marked);
+        if (first) more = attend_tile<DT, DT == NSN_DTYPE_BF16>(p, stg, again, kvh, start, n, z, marked, written);
+        else more = attend_tile<DT, false>(p, stg, again, kvh, start, n, z, marked, written);
         more = more && !marked;
     }
 }
@@ -480,6 +488,17 @@ extern "C" int nsn_prompt_attention(const nsn_prompt_args *a, nsn_stream_t strea
     if (a->tokens > 0x7fffffff || a->seqs > 0x7fffff00 || group > kRows * kMaxGrid / a->tokens) return NSN_EINVAL;
     const int64_t tiles = a->tokens * group / kRows + (a->seqs < a->tokens ? a->seqs : a->tokens);
     if (tiles > kMaxGrid / a->heads_kv) return NSN_EINVAL;   // (more rows than memory holds)
+    // the output in the queries' place, row for row, or apart from all inputs
+    const uintptr_t lo = reinterpret_cast<uintptr_t>(a->out), hi = lo + a->tokens * a->heads_q * kDim * 2;
+    auto meets = [&](const void *x, int64_t heads, int64_t ts, int64_t hs) {
+        return rows_meet(reinterpret_cast<uintptr_t>(x), a->tokens, heads, 2 * ts, 2 * hs, kDim * 2, lo, hi);
+    };
+    const bool in_place = a->q == a->out && (a->tokens == 1 || a->q_token_stride == a->heads_q * kDim) &&
+                          (a->heads_q == 1 || a->q_head_stride == kDim);
+    if ((!in_place && meets(a->q, a->heads_q, a->q_token_stride, a->q_head_stride)) ||
+        meets(a->k, a->heads_kv, a->k_token_stride, a->k_head_stride) ||
+        meets(a->v, a->heads_kv, a->v_token_stride, a->v_head_stride))
+        return NSN_EINVAL;
     PromptParams p{};
     p.q = static_cast<const uint16_t *>(a->q);
     p.k = static_cast<const uint16_t *>(a->k);

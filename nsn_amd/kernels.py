@@ -589,8 +589,8 @@ def prompt_attention(q, k, v, cu_seqlens, *, scale=SCALE, status=None, check=Tru
     h // (Hq // Hkv).  Rows may be strided (slices of one fused QKV
     projection), the 128 channels contiguous.  Sequences may be empty.
     Returns out [N, Hq, 128]; rows outside every sequence are left as they
-    were in ``out`` (undefined where it is not given), and ``out`` must not
-    share memory with k and v.  What a token's K and V hold, inf and NaN included,
+    were in ``out`` (undefined where it is not given).  ``out`` may be a
+    contiguous q itself; otherwise it shares no row with q, k and v.  What a token's K and V hold, inf and NaN included,
     reaches the queries from it on only.  No gradient.  bf16 weights are
     rounded once, except for the first 64 queries of a sequence, whose few
     weights enter as hi + lo (~2^-17).  ``check`` reads the offsets and the
@@ -616,7 +616,8 @@ def prompt_attention(q, k, v, cu_seqlens, *, scale=SCALE, status=None, check=Tru
     if check:
         cu = cu_seqlens.cpu().numpy().astype(np.int64)
         require(cu[0] >= 0 and cu[-1] <= qs[0] and np.all(np.diff(cu) >= 0), "Sequence offsets")
-    if out is None:
+    given = out is not None
+    if not given:
         out = torch.empty(qs, dtype=dt, device=q.device)
     else:
         require(out.shape == qs and out.dtype == dt and out.is_contiguous() and out.get_device() == dev,
@@ -626,6 +627,7 @@ def prompt_attention(q, k, v, cu_seqlens, *, scale=SCALE, status=None, check=Tru
                         qs[1], ks[1], *_row_strides(q), *_row_strides(k), *_row_strides(v), cu_seqlens.data_ptr(),
                         scale, out.data_ptr(), st.data_ptr())
     rc = _lib.lib().nsn_prompt_attention(a, _dev.stream())
+    require(not (given and rc == _lib.NSN_EINVAL), "Output shares rows with k, v or q (it may be a contiguous q itself)")
     _lib.check(rc, "nsn_prompt_attention")
     if check and status is None:
         s = _dev.read_status(st)

@@ -59,3 +59,47 @@ def test_offsets_that_leave_the_rows_leave_one_sequence_out():
         assert torch.equal(out[rows], want[rows])
         out[rows] = 9.0
         assert bool((out == 9).all())
+
+
+@pytest.mark.parametrize("dt", [torch.float16, torch.bfloat16], ids=["fp16", "bf16"])
+@pytest.mark.parametrize("hq,hkv", [(8, 8), (16, 4), (5, 1)])
+def test_the_output_may_take_the_queries_place(hq, hkv, dt):
+    """Over clean values, and where later tokens hold inf and NaN: those tiles are computed twice."""
+    from nsn_amd import kernels
+    lens = [230, 1, 400, 64]
+    for at in (None, 63, 150, 229, 500):
+        q, k, v, cu = make(lens, hq, hkv, dt, 34)
+        if at is not None:
+            v[at, :, 5], v[at, :, 77], k[at + 1, 0, 9] = float("inf"), float("nan"), float("nan")
+        st, again = (torch.zeros(1, dtype=torch.int32, device="cuda") for _ in range(2))
+        want = kernels.prompt_attention(q, k, v, cu, status=st, check=False)
+        got = kernels.prompt_attention(q, k, v, cu, status=again, check=False, out=q)
+        assert got.data_ptr() == q.data_ptr()
+        assert torch.equal(got.view(torch.int16), want.view(torch.int16)) and torch.equal(st, again)
+        assert bool(torch.isfinite(want).all()) == (at is None)
+
+
+def test_outputs_beside_and_inside_the_inputs():
+    from nsn_amd import kernels
+    from nsn_amd.errors import IntegrityError
+    lens, hq, hkv = [100, 28], 4, 2
+    q, k, v, cu = make(lens, hq, hkv, torch.float16, 35)
+    want = kernels.prompt_attention(q, k, v, cu)
+    # right behind the queries, and in a gap of strided keys
+    room = torch.empty((2 * 128, hq, 128), dtype=torch.float16, device="cuda")
+    room[:128] = q
+    assert torch.equal(kernels.prompt_attention(room[:128], k, v, cu, out=room[128:]), want)
+    wide = torch.zeros(128 * (1 << 17), dtype=torch.float16, device="cuda")
+    k2 = wide.as_strided((128, hkv, 128), (1 << 17, 128, 1))
+    k2.copy_(k)
+    gap = wide[256:256 + q.numel()].view(q.shape)
+    assert torch.equal(kernels.prompt_attention(q, k2, v, cu, out=gap), want)
+    # rows shared with an input
+    room[1:129] = q
+    for a, b, c, out in ((room[1:129], k, v, room[:128]), (q, k2, v, wide[:q.numel()].view(q.shape))):
+        with pytest.raises(IntegrityError, match="shares rows"):
+            kernels.prompt_attention(a, b, c, cu, out=out)
+    same = make(lens, 4, 4, torch.float16, 36)
+    for out in same[1:3]:
+        with pytest.raises(IntegrityError, match="shares rows"):
+            kernels.prompt_attention(*same, out=out)
