@@ -23,8 +23,9 @@
 //
 // Values that are not finite behind a query (padding, a poisoned later token)
 // would reach it as 0 times inf: a tile whose output is not finite is done once
-// more with such values marked (output_marked).  Finite data pays one barrier a
-// tile for it; looking at V's diagonal blocks instead cost 4 % of the ragged case.
+// more with such values marked (output_marked).  Finite data pays one barrier and
+// one look at its output a tile for it; looking at V's diagonal blocks instead
+// cost 4 % of the ragged case.
 //
 // What bounds it.  Four prompts of 8192 tokens, 16 heads: 1050 to 1079 us, 1047 to
 // 1020 TFLOP/s (a 16384^3 library product reaches 1345 on this card); 16 ragged
@@ -284,7 +285,8 @@ __device__ __forceinline__ bool attend_tile(const PromptParams &p, uint8_t (&stg
         mx = halves_max(mx) * p.qscale;   // (the queries stay exact: scores scale here and inside the exponent)
         if (__builtin_amdgcn_ballot_w64(mx > m_run + kLazy)) {
             const float mnew = fmaxf(m_run, mx);
-            const float alpha = (m_run == -INFINITY) ? 0.f : __builtin_amdgcn_exp2f(m_run - mnew);
+            float alpha = (m_run == -INFINITY) ? 0.f : __builtin_amdgcn_exp2f(m_run - mnew);
+            if (marked) alpha = fmaxf(alpha, 0x1p-126f);   // (an inf stays one: no 0 times it)
             lsum *= alpha;
 #pragma unroll
             for (int ct = 0; ct < 4; ++ct) acc[ct] *= alpha;
@@ -341,9 +343,10 @@ __device__ __forceinline__ bool attend_tile(const PromptParams &p, uint8_t (&stg
 
     // The mask takes a token out of the scores; its weight is an exact 0, and 0
     // times a finite value adds nothing, but times inf or NaN it would.  Here such
-    // a value leaves the product, and a second one adds (bf16's largest)^2, past
-    // fp32's range, for every one that a row attends.  Only a tile whose output was
-    // not finite takes this path, a second time through its blocks.
+    // a value leaves the product, and for every row that attends it further ones
+    // add (bf16's largest)^2, past fp32's range: once with its sign for an inf
+    // (whatever its weight, which is positive), with both for a NaN.  Only a tile
+    // whose output was not finite takes this path, a second time through its blocks.
     auto output_marked = [&](int j) __attribute__((always_inline)) {
         const uint8_t *vj = stg[j % kStages];
         int lim = qi - j * kBlockTok;
@@ -355,13 +358,17 @@ __device__ __forceinline__ bool attend_tile(const PromptParams &p, uint8_t (&stg
                 __builtin_amdgcn_sched_barrier(0);
                 const u32x2 a0 = read_column(vj + vx[ct] + 4096 * c);
                 const u32x2 a1 = read_column(vj + (vx[ct] ^ 32) + 4096 * c + 2048);
-                u32x4 a = {a0[0], a0[1], a1[0], a1[1]}, mark, attended;
+                u32x4 a = {a0[0], a0[1], a1[0], a1[1]}, plus, minus, attended;
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    const u16x2 past = __builtin_elementwise_sub_sat(__builtin_bit_cast(u16x2, a[e] & 0x7fff7fffu),
+                    const uint32_t pair = a[e];
+                    const u16x2 past = __builtin_elementwise_sub_sat(__builtin_bit_cast(u16x2, pair & 0x7fff7fffu),
                                                                      u16x2{kInf<DT> - 1, kInf<DT> - 1});
                     const u16x2 one = __builtin_elementwise_min(past, u16x2{1, 1});   // 1 where not finite
-                    mark[e] = __builtin_bit_cast(uint32_t, one * u16x2{kLargest, kLargest});
+                    const u16x2 nan = __builtin_elementwise_min(past - one, u16x2{1, 1});
+                    const u16x2 negative = __builtin_bit_cast(u16x2, pair) >> u16x2{15, 15};
+                    plus[e] = __builtin_bit_cast(uint32_t, (one & (nan | (negative ^ u16x2{1, 1}))) * u16x2{kLargest, kLargest});
+                    minus[e] = __builtin_bit_cast(uint32_t, (one & (nan | negative)) * u16x2{kLargest | 0x8000, kLargest | 0x8000});
                     a[e] &= __builtin_bit_cast(uint32_t, one - u16x2{1, 1});
                     const int i = 8 * (c & 1) + 2 * e, t = 32 * (c >> 1) + 8 * (i >> 2) + 4 * h + (i & 3);
                     attended[e] = (t <= lim ? kLargest : 0u) | (t + 1 <= lim ? uint32_t{kLargest} << 16 : 0u);
@@ -369,7 +376,8 @@ __device__ __forceinline__ bool attend_tile(const PromptParams &p, uint8_t (&stg
                 acc[ct] = mfma<DT>(a, pb[c], acc[ct]);
                 if constexpr (LO) acc[ct] = mfma<DT>(a, pl[c], acc[ct]);
                 asm volatile("" : "+v"(lim));
-                acc[ct] = mfma<NSN_DTYPE_BF16>(mark, attended, acc[ct]);
+                acc[ct] = mfma<NSN_DTYPE_BF16>(plus, attended, acc[ct]);
+                acc[ct] = mfma<NSN_DTYPE_BF16>(minus, attended, acc[ct]);
             }
         }
     };
@@ -385,13 +393,13 @@ __device__ __forceinline__ bool attend_tile(const PromptParams &p, uint8_t (&stg
         __builtin_amdgcn_sched_barrier(0);
     };
     int j = 0;
-    for (; !LO && j < jfull; ++j) {   // (a tile of first queries has at most one such block a wave)
+    for (; !LO && !marked && j < jfull; ++j) {   // (a tile of first queries has at most one such block a wave)
         begin(j);
         scores(j);
         softmax(j, false);
         output(j);
     }
-    for (; j < nblk; ++j) {   // the diagonal (a loop of its own: the other one carries no mask)
+    for (; j < nblk; ++j) {   // the diagonal (a loop of its own: the other one carries no mask), all blocks of a marked tile
         begin(j);
         if (j >= jend) continue;
         scores(j);

@@ -591,7 +591,8 @@ def prompt_attention(q, k, v, cu_seqlens, *, scale=SCALE, status=None, check=Tru
     Returns out [N, Hq, 128]; rows outside every sequence are left as they
     were in ``out`` (undefined where it is not given).  ``out`` may be a
     contiguous q itself; otherwise it shares no row with q, k and v.  What a token's K and V hold, inf and NaN included,
-    reaches the queries from it on only.  No gradient.  bf16 weights are
+    reaches the queries from it on only: an inf in V as an inf of its sign,
+    whatever its weight, a NaN or both signs as a NaN.  No gradient.  bf16 weights are
     rounded once, except for the first 64 queries of a sequence, whose few
     weights enter as hi + lo (~2^-17).  ``check`` reads the offsets and the
     status word back and raises; without it offsets that leave the rows set

@@ -103,3 +103,64 @@ def test_outputs_beside_and_inside_the_inputs():
     for out in same[1:3]:
         with pytest.raises(IntegrityError, match="shares rows"):
             kernels.prompt_attention(*same, out=out)
+
+
+def classes(v, at, n, hq):
+    """[n, hq, 128] of what values past fp32 leave of the outputs: 0 finite, 1 inf, -1 -inf, 2 NaN, by a running scan."""
+    x = v[at:at + n].repeat_interleave(hq // v.shape[1], 1)
+    plus, minus, nan = ((f.cumsum(0) > 0) for f in (x == float("inf"), x == float("-inf"), torch.isnan(x)))
+    out = plus.int() - minus.int()
+    out[nan | (plus & minus)] = 2
+    return out
+
+
+def classes_of(out):
+    c = (out == float("inf")).int() - (out == float("-inf")).int()
+    c[torch.isnan(out)] = 2
+    return c
+
+
+INF, NAN = float("inf"), float("nan")
+
+
+@pytest.mark.parametrize("dt", [torch.float16, torch.bfloat16], ids=["fp16", "bf16"])
+@pytest.mark.parametrize("hq,hkv", [(8, 8), (16, 4), (5, 1)])
+@pytest.mark.parametrize("marks", [
+    [(0, 3, INF), (0, 4, -INF), (0, 5, NAN)], [(70, 3, -INF)], [(229, 3, -INF)],
+    [(20, 3, INF), (90, 3, INF), (200, 3, -INF), (10, 40, -INF), (11, 40, INF), (64, 41, -INF), (300, 41, NAN)],
+    [(63, 9, -INF), (64, 9, -INF), (63, 10, NAN), (128, 11, INF), (129, 12, -INF), (191, 13, NAN), (192, 14, -INF)]],
+    ids=["first", "middle", "last", "several", "borders"])
+@pytest.mark.parametrize("sharp", [False, True])
+def test_an_attended_value_past_the_numbers_keeps_its_sign_and_kind(marks, hq, hkv, dt, sharp):
+    """An inf in V is an inf of its sign in every output that attends it, whatever its
+    weight, a NaN (or both signs) a NaN: in the query's own block and in later ones."""
+    from nsn_amd import kernels
+    lens = [320, 20]
+    q, k, v, cu = make(lens, hq, hkv, dt, 37)
+    if sharp:
+        q = q * 60       # most weights are below 2^-149
+    clean = kernels.prompt_attention(q, k, v, cu)
+    for tok, ch, x in marks:
+        v[tok, :, ch] = x
+    st = torch.zeros(1, dtype=torch.int32, device="cuda")
+    out = kernels.prompt_attention(q, k, v, cu, status=st, check=False)
+    want = torch.cat([classes(v, 0, 320, hq), classes(v, 320, 20, hq)])
+    assert torch.equal(classes_of(out), want.int())
+    assert torch.equal(out[want == 0], clean[want == 0])
+
+
+@pytest.mark.parametrize("dt", [torch.float16, torch.bfloat16], ids=["fp16", "bf16"])
+def test_an_inf_survives_larger_scores_behind_it(dt):
+    """Token 1's weight falls past fp32's range when token 150's score is seen, three blocks on."""
+    from nsn_amd import kernels
+    q, k, v, cu = make([200], 4, 2, dt, 38)
+    q[:] = 8.0
+    k[:] = 0.0
+    k[150] = 8.0          # a score of 128 * 64 * scale = 724
+    clean = kernels.prompt_attention(q, k, v, cu)
+    v[1, :, 2], v[1, :, 3] = -INF, INF
+    st = torch.zeros(1, dtype=torch.int32, device="cuda")
+    out = kernels.prompt_attention(q, k, v, cu, status=st, check=False)
+    want = classes(v, 0, 200, 4)
+    assert torch.equal(classes_of(out), want)
+    assert torch.equal(out[want == 0], clean[want == 0])
