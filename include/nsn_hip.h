@@ -367,9 +367,10 @@ int nsn_prompt_attention(const nsn_prompt_args *args, nsn_stream_t stream);
  * NSN_ST_EMPTY.  Nonfinite queries or own tail tokens raise
  * NSN_ST_NONFINITE_ATTN_INPUT, a nonfinite output NSN_ST_NONFINITE_OUTPUT;
  * block counts that differ or pass a capacity raise NSN_ST_CAPACITY (and are
- * not read).  The prefix's K and V directions m + s*z and the softmax weights
- * times the V factor are rounded to fp16 (2^-11), everything else is fp32;
- * scales below 1/2 (an encoder's are at most 2/7).  workspace:
+ * not read).  The prefix's K and V directions m + s*z are rounded to fp16
+ * (2^-11 of themselves or 2^-17) and so are the softmax weights times the V
+ * factor (2^-11 of themselves or 2^-36 of the query row's largest), everything
+ * else is fp32; scales below 1/2 (an encoder's are at most 2/7).  workspace:
  * nsn_shared_prefix_workspace_floats(...) floats, 16-byte aligned, of this
  * call alone until it has run; n_splits as for NSN_ATTN_FAST, prefix_splits
  * any count (nsn_shared_prefix_splits gives the one that fills the GPU).

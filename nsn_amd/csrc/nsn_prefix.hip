@@ -27,8 +27,8 @@
 //     bf16 and fp16 queries enter exactly (values below 2^-29 of their row's
 //     largest lose bits);
 //   - the token factor f_K multiplies the fp32 score, f_V the softmax weight,
-//     which is then rounded to fp16 once (2^-11) against a running power of
-//     two near f_V; sums and the softmax state are fp32;
+//     which is then rounded to fp16 once: to 2^-11, or 2^-36 of the row's largest
+//     product so far (see kTop); sums and the softmax state are fp32;
 //   - V is dequantised like K into the A operand of O^T += V^T P^T: a lane holds
 //     4 channels and, per product, 8 tokens in the order of S^T's registers.
 // One dequantised operand feeds NT products (two: 32 rows more cost the softmax
@@ -124,6 +124,16 @@ constexpr int kDown = 7;
 __device__ __forceinline__ uint32_t dequant(uint32_t codes, f16x2 s, f16x2 m) {
     return as_u(__builtin_elementwise_fma(as_h2(codes), s, m));
 }
+
+// The unit 2^off in which a row's softmax weights are held.  A weight times f_V
+// is rounded to fp16.  The largest such product is put into [2^11, 2^12) (kTopTo)
+// when it passes 2^15 (kTop), the first one above 0 at once: a rounding is then
+// 2^-11 of its product or 2^-36 of the row's largest, whatever V holds at tokens
+// that the row does not attend.  The weights alone stay in fp32's range by their
+// scores: they are put to 2^36 when they pass 2^60, which leaves room for any f_V
+// of an encoder (2^-25 to 2^17); a first product below 2^-30 counts as that.
+constexpr float kTop = 32768.f, kScoreMax = 60.f, kScoreTo = 36.f;
+constexpr int kTopTo = 11, kLeast = -30;
 
 // 4 channels of tokens a (low half) and b (high half), given each token's
 // 4 * BITS code bits in the low bits of a word: channel c at bit kV4[c].
@@ -253,19 +263,21 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(2))
     }
     __syncthreads();
 
-    float c1[NT], m_run[NT], lsum[NT];
+    // acc and lsum hold weights times 2^-off: a power of two of its own for each row,
+    // as far below the largest weight times f_V seen as fp16 allows (see kTop)
+    float c1[NT], off[NT], top[NT], lsum[NT];
     f32x16 acc[NT][4];   // O^T: register i of tile ct is channel 4 (8 (i / 4) + 4 h + i % 4) + ct of the lane's row
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
         c1[nt] = c1_s[32 * nt + col];
-        m_run[nt] = -INFINITY;
+        off[nt] = -INFINITY;
+        top[nt] = 0.f;
         lsum[nt] = 0.f;
 #pragma unroll
         for (int ct = 0; ct < 4; ++ct)
 #pragma unroll
             for (int i = 0; i < 16; ++i) acc[nt][ct][i] = 0.f;
     }
-    int e_run = -1000;   // acc and lsum hold weights times 2^-e_run: times f_V below 2^12
 
     // where channels 2 l, 2 l + 1 of the K scales and mins go in operand order
     int kpos[2];
@@ -314,22 +326,6 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(2))
                 const _Float16 four = static_cast<_Float16>(4.f), down = static_cast<_Float16>(1.f / (1 << kDown));
                 vs[c] = as_h2(perm(sw, sw, sel)) * f16x2{up, up} * f16x2{four, four};   // (up * 4 is past fp16's range)
                 vm[c] = as_h2(perm(mw, mw, sel)) * f16x2{down, down};
-            }
-            // the block's largest f_V < 2^e
-            const float fv = *reinterpret_cast<const float *>(mt + S::VF + 4 * l);
-            int e = ((wave::wave_max(static_cast<int32_t>(__float_as_uint(fv) & 0x7fffffffu)) >> 23) & 255) - 126;
-            e = e < -100 ? -100 : (e > 100 ? 100 : e);
-            if (e > e_run + 4) {   // (uniform)
-                if (e_run > -1000) {
-                    const float down = ldexpf(1.f, e_run - e);
-#pragma unroll
-                    for (int nt = 0; nt < NT; ++nt) {
-                        lsum[nt] *= down;
-#pragma unroll
-                        for (int ct = 0; ct < 4; ++ct) acc[nt][ct] *= down;
-                    }
-                }
-                e_run = e;
             }
             asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // (the operand-order K scales, this wave's own)
         }
@@ -391,7 +387,7 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(2))
             const float a0 = max3f(s[nt][0], s[nt][1], s[nt][2]), a1 = max3f(s[nt][3], s[nt][4], s[nt][5]);
             const float a2 = max3f(s[nt][6], s[nt][7], s[nt][8]), a3 = max3f(s[nt][9], s[nt][10], s[nt][11]);
             const float a4 = max3f(s[nt][12], s[nt][13], s[nt][14]);
-            mx[nt] = halves_max(max3f(max3f(a0, a1, a2), max2f(a3, a4), s[nt][15])) * c1[nt];
+            mx[nt] = max3f(max3f(a0, a1, a2), max2f(a3, a4), s[nt][15]) * c1[nt];   // (of the lane's half of the tokens)
         }
         // the V words of 16 tokens: lane's tokens 16 c + 4 h .. + 3 and 16 c + 8
         // + 4 h .. + 3 of the half, two dwords each; the first 16 behind the
@@ -414,33 +410,50 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(2))
                 fetch_v(0);
                 __builtin_amdgcn_sched_barrier(0);
             }
-            if (__builtin_amdgcn_ballot_w64(mx[nt] > m_run[nt] + kLazy)) {
-                const float mnew = fmaxf(m_run[nt], mx[nt]);
-                if (g > 2 * b0) {   // (nothing to scale in the first half)
-                    const float alpha = (m_run[nt] == -INFINITY) ? 0.f : __builtin_amdgcn_exp2f(m_run[nt] - mnew);
-                    lsum[nt] *= alpha;
+            auto rescale = [&](float to) __attribute__((always_inline)) {   // to: -inf only where off is
+                const float r = off[nt] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(off[nt] - to);
+                off[nt] = to;
+                lsum[nt] *= r;
+                if (g > 2 * b0) {   // (no sums in the first half)
 #pragma unroll
-                    for (int ct = 0; ct < 4; ++ct) acc[nt][ct] *= alpha;
+                    for (int ct = 0; ct < 4; ++ct) acc[nt][ct] *= r;
                 }
-                m_run[nt] = mnew;
+                return r;
+            };
+            if (__builtin_amdgcn_ballot_w64(mx[nt] > off[nt] + kScoreMax)) {
+                const float both = halves_max(mx[nt]);
+                rescale(both > off[nt] + kScoreMax ? both - kScoreTo : off[nt]);
             }
-            const float msafe = (m_run[nt] == -INFINITY ? 0.f : m_run[nt]) + static_cast<float>(e_run);
+            const float o = off[nt] == -INFINITY ? 0.f : off[nt];
             float ls[2] = {0.f, 0.f};
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                const float w = __builtin_amdgcn_exp2f(__builtin_fmaf(s[nt][i], c1[nt], -o));
+                ls[i & 1] += w;
+                s[nt][i] = w * fv[i];
+            }
+            lsum[nt] += ls[0] + ls[1];
+            float x;
+            {
+                const float a0 = max3f(s[nt][0], s[nt][1], s[nt][2]), a1 = max3f(s[nt][3], s[nt][4], s[nt][5]);
+                const float a2 = max3f(s[nt][6], s[nt][7], s[nt][8]), a3 = max3f(s[nt][9], s[nt][10], s[nt][11]);
+                const float a4 = max3f(s[nt][12], s[nt][13], s[nt][14]);
+                x = max3f(max3f(a0, a1, a2), max2f(a3, a4), s[nt][15]);
+            }
+            if (__builtin_amdgcn_ballot_w64(x > top[nt])) {
+                x = halves_max(x);
+                const bool over = x > top[nt];
+                int e = static_cast<int>(__float_as_uint(x) >> 23) - 127;   // x in [2^e, 2^(e + 1))
+                e = e < kLeast ? kLeast : e;
+                const float r = rescale(over ? off[nt] + static_cast<float>(e - kTopTo) : off[nt]);
+                top[nt] = over ? kTop : top[nt];
+#pragma unroll
+                for (int i = 0; i < 16; ++i) s[nt][i] *= r;
+            }
 #pragma unroll
             for (int c = 0; c < 2; ++c)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    float w[2];
-#pragma unroll
-                    for (int x = 0; x < 2; ++x) {
-                        const int i = 8 * c + 2 * e + x;
-                        w[x] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[nt][i], c1[nt], -msafe));
-                        ls[x] += w[x];
-                        w[x] *= fv[i];
-                    }
-                    pb[nt][c][e] = pk<NSN_DTYPE_F16>(w[0], w[1]);
-                }
-            lsum[nt] += ls[0] + ls[1];
+                for (int e = 0; e < 4; ++e) pb[nt][c][e] = pk<NSN_DTYPE_F16>(s[nt][8 * c + 2 * e], s[nt][8 * c + 2 * e + 1]);
         }
         __builtin_amdgcn_sched_barrier(0);
         // ---- O^T += V^T P^T, two steps of 16 tokens
@@ -472,8 +485,8 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(2))
     float2 *ml = reinterpret_cast<float2 *>(smem);
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
-        const float lt = halves_sum(lsum[nt]) * ldexpf(1.f, e_run);
-        if (h == 0) ml[wave * L::ROWS + 32 * nt + col] = float2{m_run[nt], lt};
+        const float lt = halves_sum(lsum[nt]);
+        if (h == 0) ml[wave * L::ROWS + 32 * nt + col] = float2{off[nt], lt};
     }
     __syncthreads();
 #pragma unroll
@@ -481,7 +494,7 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(2))
         float M = -INFINITY;
 #pragma unroll
         for (int w = 0; w < kWaves; ++w) M = fmaxf(M, ml[w * L::ROWS + 32 * nt + col].x);
-        const float a = (m_run[nt] == -INFINITY) ? 0.f : __builtin_amdgcn_exp2f(m_run[nt] - M) * ldexpf(1.f, e_run + kDown);
+        const float a = (off[nt] == -INFINITY) ? 0.f : __builtin_amdgcn_exp2f(off[nt] - M) * (1 << kDown);
 #pragma unroll
         for (int ct = 0; ct < 4; ++ct) acc[nt][ct] *= a;
     }

@@ -412,9 +412,11 @@ def shared_prefix_attention(q, prefix_k: PackedKV, prefix_v: PackedKV, k: Packed
     ``max_seq_len`` bounds the own lengths, ``max_prefix_blocks`` (default: the
     capacity) only chooses how the prefix is split.  ``check`` syncs and raises on
     nonfinite or inconsistent data; ``validate_lengths`` as in
-    ``decode_attention``.  The prefix's directions m + s*z and the softmax weights are
-    rounded to fp16 once each, as chunked prefill rounds them (a prefix token's
-    score moves by at most 2^-11 of sum |q k|; own tokens are decode_attention's).
+    ``decode_attention``.  The prefix's directions m + s*z and its softmax weights times
+    the V factor are rounded to fp16 once each: a direction by 2^-11 of itself or 2^-17
+    (a prefix token's score moves by at most 2^-11 of sum |q k|, or 2^-17 of f_K sum |q|),
+    a weighted factor by 2^-11 of itself or 2^-36 of its query row's largest.  Own tokens
+    are decode_attention's, so a whole cache there is answered more exactly.
     The reference's decode reads a whole cache per sequence
     (loop_kv_vf01_kernel.py:56-139).
     """
