@@ -40,6 +40,11 @@ def stream():
     return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device())
 
 
+def capturing():
+    """Work of the current stream is recorded into a HIP graph, not run."""
+    return torch.cuda.is_current_stream_capturing()
+
+
 def ptr(t):
     return None if t is None else t.data_ptr()
 

@@ -358,14 +358,14 @@ class PackedKVCache(Cache):
     def attend(self, slot, q, scale):
         """Decode attention of q [B, Hq, 128] over the slot by the cache's arm
         (not NATIVE); returns the bf16 output [B, Hq, 128]."""
-        L = self.store.length[slot]
         kside, vside = self.store.side(slot, "K"), self.store.side(slot, "V")
-        seq = self.store.lengths(slot)
         if self.graph_mode:
             # lengths from the device counters, the capacity as the bound: no
             # launch argument changes from step to step
             require(self.arm == "PACKED_KV_FUSED" and not self.strict, "Device positions: fused arm, strict=False")
             L, seq = self.cap_len, self.counters[:self.batch]
+        else:
+            L, seq = self.store.length[slot], self.store.lengths(slot)
         kw = dict(max_seq_len=L, scale=scale, check=self.strict, status=None if self.strict else self.status)
         if self.arm == "PACKED_GROUPED":
             vd = PackedKV(None, None, None, None, None, None, self.materialize(slot, "V", self.tail_dtype), kside.bits)

@@ -84,6 +84,7 @@ class StreamingKVCache:
         self.block_cap = max(1, max_tokens // BLOCK)
         self.tail_cap = 2 * BLOCK + max_append
         self.device = device
+        self._gpu = torch.device(device).type == "cuda"
         nbytes = BLOCK * DIM * bits // 8
         # one allocation per array for all slots ([slots, batch, heads, ...]):
         # sequences are copied over every slot by one launch
@@ -110,6 +111,7 @@ class StreamingKVCache:
         self.seq_length = [[0] * batch for _ in range(slots)]       # tokens held per slot and sequence
         self.seq_compressed = [[0] * batch for _ in range(slots)]   # of which packed
         self._len_dev = {}               # cached int32 length tensors
+        self._len_captured = {}          # of which HIP graphs read
         self.status = _dev.new_status(device)
         self.encoded_blocks = [0] * slots
         self._side = None                # second stream of the compressions
@@ -153,25 +155,42 @@ class StreamingKVCache:
 
     def length_tensor(self, L) -> torch.Tensor:
         """int32 [B] device tensor of the lengths L (an int for every sequence, or
-        one per sequence), made once per distinct value and kept."""
+        one per sequence), made once per distinct value and kept (for good, once a
+        HIP graph reads it).  What a capture makes itself is the graph's alone:
+        unset until a replay, it must not answer an eager call."""
         key = tuple(L) if isinstance(L, (list, tuple)) else (int(L),) * self.batch
         t = self._len_dev.get(key)
+        captured = self._gpu and _dev.capturing()
         if t is None:
-            # Uploaded from pinned memory without a host wait: a pageable copy
-            # would drain the stream first, so every new length (each chunk,
-            # each decode step) would leave the GPU idle while the host issues
-            # the next launches.  The oldest entries are dropped (a dropped
-            # tensor's memory is reused only by later work on the stream).
-            # One length for all -- each decode step of a uniform batch brings a
-            # new one -- is a single fill on the device instead.
-            gpu = torch.device(self.device).type == "cuda"
-            if min(key) == max(key):
-                t = torch.full((self.batch,), key[0], dtype=torch.int32, device=self.device)
-            else:
-                t = torch.tensor(key, dtype=torch.int32, pin_memory=gpu).to(self.device, non_blocking=gpu)
+            t = self._upload(key)
+            if captured:
+                return t
+            # the oldest entries are dropped (a dropped tensor's memory is
+            # reused only by later work on the stream)
             if len(self._len_dev) >= 256:
                 self._len_dev.pop(next(iter(self._len_dev)))
             self._len_dev[key] = t
+        if captured:
+            self._len_captured[key] = t
+        return t
+
+    def _upload(self, values):
+        """int32 device tensor of host integers.  Uploaded from pinned memory
+        without a host wait: a pageable copy would drain the stream first, so
+        every new length (each chunk, each decode step) would leave the GPU idle
+        while the host issues the next launches.  One value for all -- each decode
+        step of a uniform batch brings a new one -- is a single fill on the device
+        instead, and so is each run of equal values under a capture: a recorded
+        copy would read host memory that is gone by the replay."""
+        if min(values) == max(values):
+            return torch.full((len(values),), values[0], dtype=torch.int32, device=self.device)
+        if not (self._gpu and _dev.capturing()):
+            t = torch.tensor(values, dtype=torch.int32, pin_memory=self._gpu)
+            return t.to(self.device, non_blocking=self._gpu)
+        t = torch.empty(len(values), dtype=torch.int32, device=self.device)
+        cuts = [i for i in range(len(values)) if i == 0 or values[i] != values[i - 1]]
+        for i, end in zip(cuts, cuts[1:] + [len(values)]):
+            t[i:end].fill_(values[i])
         return t
 
     def tail_len(self, slot):
@@ -384,9 +403,7 @@ class StreamingKVCache:
 
     def _offsets(self, lengths):
         """Device offsets of sequences of these lengths laid end to end."""
-        gpu = torch.device(self.device).type == "cuda"
-        cu = torch.tensor([0, *accumulate(lengths)], dtype=torch.int32, pin_memory=gpu)
-        return cu.to(self.device, non_blocking=gpu)   # (from pinned memory without a host wait, like the lengths)
+        return self._upload([0, *accumulate(lengths)])
 
     # ------------------------------------------------------------------ sequences
     def _require_no_branch(self):
