@@ -38,7 +38,7 @@ from itertools import accumulate
 import torch
 
 from . import _dev, _lib
-from .errors import IntegrityError, require
+from .errors import IntegrityError, NumericalFailure, require
 from .kernels import BLOCK, DIM, PackedKV
 
 MIN_TAIL = 64
@@ -365,11 +365,16 @@ class StreamingKVCache:
             self.compress_to(s, [decode_target(L, C) for L, C in zip(self.seq_length[s], self.seq_compressed[s])])
 
     def check_status(self):
-        """Raise if any compression flagged nonfinite input or fp16 metadata trouble (syncs)."""
+        """Raise if any compression flagged nonfinite input or fp16 metadata trouble, or
+        a prompt that was given no status word a nonfinite output (syncs)."""
         s = _dev.read_status(self.status)
         if s:
             from .primitives import _encode_raise
             _encode_raise(s)
+            if s & _lib.ST_CAPACITY:
+                raise IntegrityError("Prompt offsets or tail capacity")
+            if s & _lib.ST_NONFINITE_OUTPUT:
+                raise NumericalFailure("Nonfinite prompt attention output")
 
     def prompt(self, slot, q, k, v, lengths, **kw):
         """Causal attention over whole prompts of different lengths laid end to end,
@@ -378,7 +383,8 @@ class StreamingKVCache:
         per sequence, their sum N; 0 for a sequence that takes no part).  A prompt
         sees no context: its sequence must be empty, and it must fit the tail
         (compress afterwards, with ``post_prefill``).  Returns out [N, Hq, 128];
-        ``kw`` as ``kernels.prompt_attention`` takes them."""
+        ``kw`` as ``kernels.prompt_attention`` takes them (``check=False`` without a
+        ``status``: ``check_status`` reports the flags)."""
         lengths = [int(n) for n in lengths]
         require(self.prefix is None, "A branch decodes only: prompts go to the cache it branches from")
         require(len(lengths) == self.batch and all(n >= 0 for n in lengths) and sum(lengths) == q.shape[0],
@@ -389,8 +395,10 @@ class StreamingKVCache:
             if n > self.tail_cap or n > self.block_cap * BLOCK + self.tail_cap:
                 raise IntegrityError("Tail overflow: compress before appending more tokens")
         cu = self._offsets(lengths)
-        out = _attn().prompt_attention(q, k, v, cu, **kw)
         st = kw.get("status")
+        if st is None and not kw.get("check", True):
+            st = kw["status"] = self.status
+        out = _attn().prompt_attention(q, k, v, cu, **kw)
         kt, vt = self._sides[(slot, "K")].kv.tail, self._sides[(slot, "V")].kv.tail
         rc = _lib.lib().nsn_prompt_append(
             k.data_ptr(), v.data_ptr(), _dev.dtype_code(k.dtype), k.shape[0], self.heads, *_attn()._row_strides(k),
