@@ -77,14 +77,14 @@ class StreamingKVCache:
 
     def __init__(self, slots, batch, heads, max_tokens, *, bits=3, dtype=torch.float16, max_append=512,
                  device=None):
-        device = device or torch.device("cuda:0")
+        device = torch.empty(0, device=device or torch.device("cuda:0")).device   # (with its index, however named)
         require(bits in (3, 4, 5), "Bits")
         require(dtype in (torch.float16, torch.bfloat16), "Tail dtype")
         self.slots, self.batch, self.heads, self.bits, self.dtype = slots, batch, heads, bits, dtype
         self.block_cap = max(1, max_tokens // BLOCK)
         self.tail_cap = 2 * BLOCK + max_append
         self.device = device
-        self._gpu = torch.device(device).type == "cuda"
+        self._gpu = device.type == "cuda"
         nbytes = BLOCK * DIM * bits // 8
         # one allocation per array for all slots ([slots, batch, heads, ...]):
         # sequences are copied over every slot by one launch
