@@ -374,7 +374,8 @@ int nsn_prompt_attention(const nsn_prompt_args *args, nsn_stream_t stream);
  * nsn_shared_prefix_workspace_floats(...) floats, 16-byte aligned, of this
  * call alone until it has run; n_splits as for NSN_ATTN_FAST, prefix_splits
  * any count (nsn_shared_prefix_splits gives the one that fills the GPU).
- * heads_q / heads_kv <= 8; bits 3 or 5, the same on all sides.  No counterpart
+ * heads_q / heads_kv <= 8; bits 3 or 5, the same on all sides.  out may be q's
+ * own memory, but not overlap it otherwise (NSN_EINVAL).  No counterpart
  * in the reference, whose decode reads a whole cache per sequence
  * (experiments/ac08/source/loop_kv_vf01_kernel.py:56-139).
  */

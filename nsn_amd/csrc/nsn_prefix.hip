@@ -772,6 +772,12 @@ extern "C" int nsn_shared_prefix_attention(const nsn_shared_args *a, nsn_stream_
     if (a->out_dtype != NSN_DTYPE_F16 && a->out_dtype != NSN_DTYPE_BF16) return NSN_EINVAL;
     for (const void *ptr : {a->q, static_cast<const void *>(a->out), static_cast<const void *>(a->workspace)})
         if (reinterpret_cast<uintptr_t>(ptr) & 15u) return NSN_EINVAL;
+    // the output in the queries' place, or apart from them (the joint kernel's
+    // workgroups write while others read)
+    const uintptr_t q0 = reinterpret_cast<uintptr_t>(a->q), o0 = reinterpret_cast<uintptr_t>(a->out);
+    if (a->heads_q > (1 << 23) / a->batch) return NSN_EINVAL;
+    const uintptr_t bytes = static_cast<uintptr_t>(a->batch * a->heads_q) * kDim * 2;
+    if (q0 != o0 && q0 < o0 + bytes && o0 < q0 + bytes) return NSN_EINVAL;
     for (const nsn_kv_side *s : {&a->prefix_k, &a->prefix_v}) {
         if (!s->blocks || s->block_cap <= 0 || s->block_cap > (1 << 25)) return NSN_EINVAL;
         for (const void *ptr : {static_cast<const void *>(s->codes), static_cast<const void *>(s->mins),
@@ -780,7 +786,7 @@ extern "C" int nsn_shared_prefix_attention(const nsn_shared_args *a, nsn_stream_
     }
     const int64_t group = a->heads_q / a->heads_kv, fan = a->batch / a->prefixes;
     const int64_t rows = fan * group;
-    if (rows > (1 << 24) || a->batch * a->heads_q > (1 << 23)) return NSN_EINVAL;
+    if (rows > (1 << 24)) return NSN_EINVAL;
     const int tile = row_tile(rows);
     const int64_t row_tiles = (rows + tile - 1) / tile;
     const int64_t wgs = a->prefixes * a->heads_kv * row_tiles;

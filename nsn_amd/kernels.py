@@ -386,6 +386,8 @@ def _shared_args(q, prefix_k: PackedKV, prefix_v: PackedKV, k: PackedKV, v: Pack
         out = torch.empty(shape, dtype=out_dtype, device=q.device)
     require(out.shape == shape and out.dtype == out_dtype and out.is_contiguous() and out.device == q.device,
             "Output shape/type")
+    apart = out.data_ptr() - q.data_ptr()
+    require(apart == 0 or abs(apart) >= 2 * q.numel(), "Output overlaps the queries (it may be their memory)")
     st = _dev.new_status(q.device) if status is None else _dev.require_status(status, dev)
     code = _dev.dtype_code
     a = _lib.SharedArgs(q.data_ptr(), code(q.dtype), B, Hq, Hkv, P, scale, bits, prefix_k.side(), prefix_v.side(),
@@ -405,8 +407,8 @@ def shared_prefix_attention(q, prefix_k: PackedKV, prefix_v: PackedKV, k: Packed
     prefix p; ``blocks`` [P] may be 0; their tails are not read: a prefix's tail
     tokens are its sequences' own).  k, v, seq_len: each sequence's own packed
     blocks and tail, as ``decode_attention`` takes them (0 own tokens: the prefix
-    alone).  Returns out [B, Hq, 128] in ``out_dtype`` (bf16 or fp16): the softmax
-    readout over prefix and own tokens.  All sides carry decode factors and one
+    alone).  Returns out [B, Hq, 128] in ``out_dtype`` (bf16 or fp16; q's own
+    memory, or apart from it): the softmax readout over prefix and own tokens.  All sides carry decode factors and one
     width, 3 or 5 bits; Hq // Hkv <= 8.
 
     ``max_seq_len`` bounds the own lengths, ``max_prefix_blocks`` (default: the

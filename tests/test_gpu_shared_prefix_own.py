@@ -73,3 +73,19 @@ def test_a_row_beside_an_empty_one_without_a_prefix():
             pk, pv = (PackedKV(s.codes[p:p + 1], s.norm[p:p + 1], s.min[p:p + 1], s.scale[p:p + 1], s.factor[p:p + 1],
                                s.blocks[p:p + 1], None, s.bits) for s, p in ((args[1], b // 2), (args[2], b // 2)))
             check(out[b:b + 1], (q[b:b + 1], pk, pv, args[3], args[4], seq[b:b + 1]), pick)
+
+
+@pytest.mark.parametrize("max_seq_len", [40, 2000], ids=["joint", "apart"])
+def test_the_output_may_be_the_queries_memory(max_seq_len):
+    from nsn_amd import kernels
+    from nsn_amd.errors import IntegrityError
+    args, dense = case([5, 2], [10, 20, 30, 40], 14, 2, 3, seed=24)
+    q = args[0]
+    want = kernels.shared_prefix_attention(*args, max_seq_len=max_seq_len)
+    room = torch.empty((6, 14, DIM), dtype=q.dtype, device="cuda")
+    room[1:5] = q
+    for out in (room[:4], room[2:]):
+        with pytest.raises(IntegrityError, match="overlaps"):
+            kernels.shared_prefix_attention(room[1:5], *args[1:], max_seq_len=max_seq_len, out=out)
+    got = kernels.shared_prefix_attention(*args, max_seq_len=max_seq_len, out=q)
+    assert got.data_ptr() == q.data_ptr() and torch.equal(got, want)
