@@ -433,12 +433,13 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(2))
                 s[nt][i] = w * fv[i];
             }
             lsum[nt] += ls[0] + ls[1];
-            float x;
+            float x;   // (of the lane's half of the tokens)
             {
-                const float a0 = max3f(s[nt][0], s[nt][1], s[nt][2]), a1 = max3f(s[nt][3], s[nt][4], s[nt][5]);
-                const float a2 = max3f(s[nt][6], s[nt][7], s[nt][8]), a3 = max3f(s[nt][9], s[nt][10], s[nt][11]);
-                const float a4 = max3f(s[nt][12], s[nt][13], s[nt][14]);
-                x = max3f(max3f(a0, a1, a2), max2f(a3, a4), s[nt][15]);
+                auto mag = [&](int i) { return __builtin_fabsf(s[nt][i]); };   // (a modifier of the maximum)
+                const float a0 = max3f(mag(0), mag(1), mag(2)), a1 = max3f(mag(3), mag(4), mag(5));
+                const float a2 = max3f(mag(6), mag(7), mag(8)), a3 = max3f(mag(9), mag(10), mag(11));
+                const float a4 = max3f(mag(12), mag(13), mag(14));
+                x = max3f(max3f(a0, a1, a2), max2f(a3, a4), mag(15));
             }
             if (__builtin_amdgcn_ballot_w64(x > top[nt])) {
                 x = halves_max(x);

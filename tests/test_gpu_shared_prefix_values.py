@@ -132,3 +132,24 @@ def test_scores_that_rise_and_fall_by_hundreds(hq, hkv):
         kx = kx * 0.1 + (step / 10)[None, None, :, None]
         vx *= torch.exp2((torch.arange(n, device="cuda") % 13) - 6.0)[None, None, :, None]
         run(q, kx, vx, 3, [1, 1, 2, 1, 1], 44)
+
+
+def test_factors_of_either_sign():
+    """A token's factor enters as it is: with its sign turned, in K and V, the token enters with its sign turned."""
+    from nsn_amd import kernels
+    q, kx, vx = drawn(6, 1, 4, 8, 2, 640)
+    g = torch.Generator(device="cuda").manual_seed(45)
+    pk, pkd = encode(kx.half(), 3)
+    pv, pvd = encode((vx * 300).half(), 3)
+    own = [1, 2, 3, 4]
+    k, kd = packed(g, own, 2, 3, torch.float16)
+    v, vd = packed(g, own, 2, 3, torch.float16)
+    turned = (torch.rand(640, generator=g, device="cuda") < 0.5).double()
+    for side, dense in ((pk, pkd), (pv, pvd)):
+        sign = (1 - 2 * turned).reshape(1, 1, 10, 64)
+        side.factor.mul_(sign.float())
+        dense[0] *= (1 - 2 * turned)[None, :, None]
+    seq = torch.tensor(own, dtype=torch.int32, device="cuda")
+    out = kernels.shared_prefix_attention(q.bfloat16(), pk, pv, k, v, seq)
+    pk.factor.abs_(), pv.factor.abs_()      # (the bound takes magnitudes)
+    check(out, q.bfloat16(), pk, pv, pkd, pvd, kd, vd)
