@@ -632,7 +632,8 @@ def prompt_attention(q, k, v, cu_seqlens, *, scale=SCALE, status=None, check=Tru
                         qs[1], ks[1], *_row_strides(q), *_row_strides(k), *_row_strides(v), cu_seqlens.data_ptr(),
                         scale, out.data_ptr(), st.data_ptr())
     rc = _lib.lib().nsn_prompt_attention(a, _dev.stream())
-    require(not (given and rc == _lib.NSN_EINVAL), "Output shares rows with k, v or q (it may be a contiguous q itself)")
+    require(not (given and rc == _lib.NSN_EINVAL),
+            "Output is not 16-byte aligned, or shares rows with k, v or q (it may be a contiguous q itself)")
     _lib.check(rc, "nsn_prompt_attention")
     if check and status is None:
         s = _dev.read_status(st)
