@@ -110,7 +110,7 @@ class StreamingKVCache:
                 self._sides[(s, name)] = _Side(kv, w["headers"][s])
         self.seq_length = [[0] * batch for _ in range(slots)]       # tokens held per slot and sequence
         self.seq_compressed = [[0] * batch for _ in range(slots)]   # of which packed
-        self._len_dev = {}               # cached int32 length tensors
+        self._len_dev = {}               # cached int32 length tensors: {lengths: {stream: tensor}}
         self._len_captured = {}          # of which HIP graphs read
         self.status = _dev.new_status(device)
         self.encoded_blocks = [0] * slots
@@ -155,23 +155,26 @@ class StreamingKVCache:
 
     def length_tensor(self, L) -> torch.Tensor:
         """int32 [B] device tensor of the lengths L (an int for every sequence, or
-        one per sequence), made once per distinct value and kept (for good, once a
-        HIP graph reads it).  What a capture makes itself is the graph's alone:
-        unset until a replay, it must not answer an eager call."""
+        one per sequence), made once per distinct value and stream and kept (for
+        good, once a HIP graph reads it): another stream could read it before it
+        is written.  What a capture makes itself is the graph's alone: unset until
+        a replay, it must not answer an eager call."""
         key = tuple(L) if isinstance(L, (list, tuple)) else (int(L),) * self.batch
-        t = self._len_dev.get(key)
-        captured = self._gpu and _dev.capturing()
+        kept = self._len_dev.get(key)
+        if self._gpu and _dev.capturing():
+            if not kept:
+                return self._upload(key)
+            t = self._len_captured[key] = next(iter(kept.values()))
+            return t
+        stream = _dev.stream() if self._gpu else 0
+        t = kept.get(stream) if kept else None
         if t is None:
             t = self._upload(key)
-            if captured:
-                return t
-            # the oldest entries are dropped (a dropped tensor's memory is
-            # reused only by later work on the stream)
-            if len(self._len_dev) >= 256:
+            # the oldest lengths are dropped (a dropped tensor's memory is
+            # reused only by later work on its stream)
+            if kept is None and len(self._len_dev) >= 256:
                 self._len_dev.pop(next(iter(self._len_dev)))
-            self._len_dev[key] = t
-        if captured:
-            self._len_captured[key] = t
+            self._len_dev.setdefault(key, {})[stream] = t
         return t
 
     def _upload(self, values):
