@@ -9,8 +9,8 @@
 // share a kv-head are the rows of one product, fan * G of them.  The own tokens
 // take the decode kernel's arithmetic (nsn_segment.hpp); the softmax states of
 // both (partials of maximum, weight sum and weighted values) are joined by the
-// kernel that follows.  No counterpart in the reference, whose decode reads a whole cache
-// per sequence (loop_kv_vf01_kernel.py:56-139).
+// kernel that follows.  No counterpart in the reference, whose decode reads a
+// whole cache per sequence (loop_kv_vf01_kernel.py:56-139).
 //
 // Prefix kernel.  A workgroup takes 32 * NT rows (NT 1 or 2) of one (prefix,
 // kv-head) and a share of its blocks; each of its 8 waves walks a contiguous
@@ -37,13 +37,14 @@
 // one workgroup per CU (their LDS), whatever the rows and prefixes.
 //
 // What bounds it.  16 sequences x 32:8 heads behind 32704 3-bit tokens (64 rows
-// x 511 blocks x 8 kv-heads, 30 MB): 24 us, 1.2 TB/s and 350 TFLOP/s.  Of it
-// 3.5 us are the first 32 tokens of all 2048 waves (fetched at once), 14 us
-// two blocks a wave -- VALU, about 520 instructions and 64 exponentials a half,
-// beside 32 MFMA; without the loop the call takes 13 us less, without the
-// exponentials 0.7 us -- and 5 us the join and the partials.  One loop body for
-// both halves (17 KB of code, no spills) took it from 34.7 to 25.8 us, one fma
-// instead of a multiply and an fma and reads a step ahead to 24.3.
+// x 511 blocks x 8 kv-heads, 30 MB): 25.3 us, 1.2 TB/s and 340 TFLOP/s.  Of it
+// 3.5 us are the first 32 tokens of all 2048 waves (fetched at once), 15 us
+// two blocks a wave -- about 560 VALU instructions and 64 exponentials a half
+// beside 32 MFMA, but VALU issue fills only 38 % of the launch's cycles, and the
+// first block takes twice the second's time -- and 5 us the join and the partials.
+// One loop body for both halves (17 KB of code, no spills) took it from 34.7 to
+// 25.8 us, one fma instead of a multiply and an fma and reads a step ahead to
+// 24.3; a unit of its own for each row's weights costs 0.6 to 1.
 #include "nsn_segment.hpp"
 #include "nsn_own_ranges.hpp"
 #include "nsn_tile.hpp"

@@ -27,13 +27,14 @@
 // one look at its output a tile for it; looking at V's diagonal blocks instead
 // cost 4 % of the ragged case.
 //
-// What bounds it.  Four prompts of 8192 tokens, 16 heads: 1050 to 1079 us, 1047 to
-// 1020 TFLOP/s (a 16384^3 library product reaches 1345 on this card); 16 ragged
-// prompts of 100 to 2000 tokens, 32:8 heads: 218 to 227 us, 790 to 758 TFLOP/s.  MFMA are busy 54 % of the
-// SIMDs' cycles at 1.85 GHz, VALU issue 45 %, LDS carries 32 KB of operands a
-// wave and block; left out, the K reads are worth 19 %, the DMA 15 %, the products
-// 21 %, the exponentials 5 %, the barrier 1 %.  Tiles of 256 rows on 8 waves (half
-// the DMA; the two waves of a SIMD kept half a block apart) took 1067 and 241 us.
+// What bounds it.  Four prompts of 8192 tokens, 16 heads: 1055 to 1095 us, 1042 to
+// 1004 TFLOP/s (a 16384^3 library product reaches 1345 on this card); 16 ragged
+// prompts of 100 to 2000 tokens, 32:8 heads: 219 to 229 us, 786 to 752 TFLOP/s.
+// MFMA are busy 54 % of the SIMDs' cycles at 1.8 GHz, VALU issue 46 %, LDS carries
+// 32 KB of operands a wave and block; left out, the K reads are worth 19 %, the DMA
+// 15 %, the products 21 %, the exponentials 5 %, the barrier 1 %.  Tiles of 256 rows
+// on 8 waves (half the DMA; the two waves of a SIMD kept half a block apart) took
+// 1067 and 241 us where these took 1037 and 222.
 //
 // Work: tiles are numbered by their place in their sequence, the last places
 // of all sequences first (the causal work grows with the place), and a

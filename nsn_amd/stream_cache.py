@@ -429,7 +429,10 @@ class StreamingKVCache:
 
         ``seq_length`` of a branch counts its own tokens, ``prefix_tokens`` the shared
         ones.  It appends, compresses and decodes (fast kernel) like any cache, and
-        forks among the rows of one prefix; prompts and prefill are refused.  While a
+        forks among the rows of one prefix (a row emptied there keeps the prefix);
+        prompts and prefill are refused.  Its decode holds the prefix's directions and
+        weights in fp16 (the bounds of ``kernels.shared_prefix_attention``), where
+        ``decode`` over a whole cache keeps them exact or as fp16 hi + lo.  While a
         branch lives this cache may grow, but not be reset, forked or copied into
         (its packed blocks must stay)."""
         require(fan >= 1, "Sequences per prefix")
