@@ -329,12 +329,13 @@ int nsn_prefill_attention_split(const nsn_prefill_args *args, int n_splits, floa
  * the first 64 enter as bf16 hi + lo, all others with one rounding.  A
  * nonfinite output raises NSN_ST_NONFINITE_OUTPUT (a nonfinite value reaches
  * the queries from its token on only: an inf in V as an inf of its sign,
- * whatever its weight, a NaN or both signs as a NaN); offsets that leave [0, tokens] raise
- * NSN_ST_CAPACITY and leave that sequence out, offsets that decrease that one
- * and every sequence behind it (which may repeat rows).  The strides are in
- * elements, multiples of 8 up to 2^22 (slices of a fused QKV projection work);
- * rows of 128 contiguous elements, arrays 16-byte aligned.  out may be q (its
- * rows contiguous too); otherwise it shares no row with q, k and v (NSN_EINVAL).
+ * whatever its weight, a NaN or both signs as a NaN); offsets that leave
+ * [0, tokens] raise NSN_ST_CAPACITY and leave that sequence out, offsets that
+ * decrease that one and every sequence behind it (which may repeat rows).  The
+ * strides are in elements, multiples of 8 up to 2^22 (slices of a fused QKV
+ * projection work); rows of 128 contiguous elements, arrays 16-byte aligned.
+ * out may be q (its rows contiguous too); otherwise it shares no row with q, k
+ * and v (NSN_EINVAL).
  * No counterpart in the reference, whose prompts run one sequence at a time
  * through the model's own attention
  * (experiments/ac08/source/loop_kv_ac08_attention.py:46-96).
